@@ -1,0 +1,45 @@
+"""What the tree must not hold, shown on the sources alone: each test reads the files under version control (or, where git is absent, every file of the same folders) and names
+the lines at fault.  The scans are textual, so a pattern here is spelled in a way that does not match itself."""
+import os
+import re
+import subprocess
+
+ROOT = os.path.abspath(os.path.join(os.path.dirname(__file__), ".."))
+SOURCE_SUFFIXES = (".py", ".sh", ".js", ".h", ".hip", ".cc", ".cpp", ".c", ".s", "Makefile")
+
+
+def source_files():
+    """Repository-relative paths of the sources, scripts and build files."""
+    r = subprocess.run(["git", "-C", ROOT, "ls-files", "-z"], capture_output=True, text=True)
+    if r.returncode == 0:
+        names = [n for n in r.stdout.split("\0") if n]
+    else:
+        names = []
+        for top in ("include", "oracle", "ps-signature-and-el-passo_amd", "tests", "tools"):
+            for dp, _, fs in os.walk(os.path.join(ROOT, top)):
+                names += [os.path.relpath(os.path.join(dp, f), ROOT) for f in fs]
+        names += [f for f in os.listdir(ROOT) if os.path.isfile(os.path.join(ROOT, f))]
+    return sorted(n for n in names if n.endswith(SOURCE_SUFFIXES) and os.path.exists(os.path.join(ROOT, n)))
+
+
+def hits(pattern):
+    rx = re.compile(pattern)
+    out = []
+    for n in source_files():
+        with open(os.path.join(ROOT, n), errors="replace") as f:
+            out += ["%s:%d: %s" % (n, i, ln.strip()) for i, ln in enumerate(f, 1) if rx.search(ln)]
+    return out
+
+
+def test_the_scan_sees_the_sources():
+    """An empty list of files would make every test below pass."""
+    names = source_files()
+    assert "bench.py" in names and "ps-signature-and-el-passo_amd/csrc/elp/pipeline.h" in names and "oracle/Makefile" in names
+
+
+def test_no_build_switch_ends_a_verification_early_and_no_script_reproduces_a_fault():
+    """A verification that returns before its last step accepts what it did not check, so no compile-time switch of that kind stays in the device headers; and a GPU fault whose
+    cause is known is guarded on the CPU (test_isa_hazards.py), never made to happen again by a script."""
+    assert hits(r"ELP_[B]ISECT") == []
+    assert [n for n in source_files() if re.search(r"fault_(repro|probe)", n)] == []
+    assert hits(r"[_]fault_(repro|probe)\b") == []
