@@ -129,7 +129,7 @@ def workload_config(args, world):
     A, H, B = args.attrs, args.hidden, args.batch
     return {"workload": "BASELINE.json config %d: batch of %d EL PASSO RP el_passo_verify_id per GPU, %d attributes with %d hidden, id-retrieval, "
                         "curve %s" % (args.config, B, A, H, "BN254 (the reference's actual mcl default; golden-vector pinned)" if args.curve == "bn254"
-                                      else "BLS12-381 (north-star curve; pinned by vectors of the reference's own wasm run on this curve, tests/golden/bls12_381_*.json)"),
+                                      else "BLS12-381 (checked against the big-integer model and the C oracle; parity with the reference unpinned, it runs on BN254)"),
             "baseline_config": args.config, "batch_per_gpu": B, "attrs": A, "hidden": H, "curve": args.curve.upper(), "window_bits": args.window or 8,
             "parallelism": "independent shards x%d + RCCL count all-reduce" % world}
 
@@ -555,9 +555,9 @@ def second_curve(pkg, synth, local_rank, dev, A, H, B, window):
            "roofline": {"bound": "hbm", "achieved": ach, "peak": HBM_PEAK_GBS, "unit": "GB/s", "frac": ach / HBM_PEAK_GBS, "traffic": None,
                         "kernel": "k_verify_id_paired<Paired<BLS12_381>>", "kernel_ms": float(ms.value)},
            "valu_bound": valu_bound(ctx, "verify_id_bls12_381" if (A == 8 and H == 4) else None, window, B, float(ms.value), 392),
-           "note": "BLS12-381 instantiation (14 limbs of 28 bits).  Parity: the reference's own wasm run on this curve (oracle/wasm_curve.js) produced "
-                   "tests/golden/bls12_381_*.json; model, C oracle, host build of the device code and the GPU reproduce every verdict "
-                   "(tests/test_oracle_bls_golden.py, tests/test_gpu_bls_golden.py); hashAndMapToG1 is mcl's (SHA-512 setHashOf, SvdW, cofactor)"}
+           "note": "BLS12-381 instantiation (14 limbs of 28 bits).  Checked against two independent implementations, the big-integer model and the C oracle "
+                   "(tests/test_oracle_bls.py, tests/test_gpu_bls.py); parity with the reference is unpinned on this curve, since the reference runs on BN254; "
+                   "hashAndMapToG1 follows mcl's construction (SHA-512 setHashOf, SvdW, cofactor)"}
     tf = os.path.join(ROOT, "profiles", "hbm_traffic_bls12_381.json")      # per-launch HBM bytes of the round's separate --pmc passes over this kernel
     if os.path.exists(tf):
         try:
@@ -570,7 +570,7 @@ def second_curve(pkg, synth, local_rank, dev, A, H, B, window):
         ncore = usable_cores()
         res["cpu_baseline"] = cpu_baseline(wl, ctx, recs, rsz, mask, flags, min(B, max(768, 24 * ncore)), bls=True)
         res["cpu_baseline"]["kind"] = "port"
-        res["cpu_baseline"]["note"] = "the C oracle's BLS12-381 build (reference structure), pinned to the reference's wasm run on this curve by tests/test_oracle_bls_golden.py"
+        res["cpu_baseline"]["note"] = "the C oracle's BLS12-381 build (reference structure), tied to the big-integer model by tests/test_oracle_bls.py"
     except Exception as e:  # pragma: no cover
         res["cpu_baseline"] = {"error": str(e)}
     try:     # aggregated verification of the same batch (round 6: main kernel on lane pairs, k_verify_id_agg_paired); the last of four calls timed with HIP events

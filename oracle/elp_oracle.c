@@ -26,11 +26,10 @@
  *
  * Second build, -DELPO_BLS12_381 (libelp_oracle_bls.so): the same restatement over BLS12-381 (6 x 64-bit limbs, y^2 = x^3 + 4, M-type twist
  * y^2 = x^3 + 4 xi, Miller loop over |z| = 0xd201000000010000, final exponentiation by the Hayashida-Hayasaka-Teruya chain AND, as a
- * self-check, by plain square-and-multiply with the integer (p^4-p^2+1)/r).  Pinning: the reference's prebuilt wasm is mcl built with
- * MCL_MAX_BIT_SIZE=384 (/root/reference/Makefile:65); with mcl's default CurveParam overwritten in its linear memory before initPairing()
- * (oracle/wasm_curve.js) it runs the whole protocol on BLS12-381, and tests/test_oracle_bls_golden.py checks this build against every vector
- * so produced (tests/golden/bls12_381_*.json): verdicts of the RP and IdP modules, hashAndMapToG1 as mcl defines it for this curve (SHA-512
- * Fp::setHashOf, Shallue-van de Woestijne map with b = 4, cofactor (z-1)^2/3) and mcl's GLV G1::mul on points outside G1.
+ * self-check, by plain square-and-multiply with the integer (p^4-p^2+1)/r).  hashAndMapToG1 follows mcl's construction for this
+ * curve (SHA-512 Fp::setHashOf, Shallue-van de Woestijne map with b = 4, cofactor (z-1)^2/3), G1::mul its GLV method on points outside G1.
+ * Pinning: none to the reference, which runs on BN254 only; tests/test_oracle_bls.py ties this build to the independent big-int model, and
+ * tests/test_oracle_bls_golden.py holds both to the recorded regression vectors tests/golden/bls12_381_*.json.
  */
 #include <stdint.h>
 #include <stdlib.h>
@@ -543,8 +542,8 @@ DEFINE_GROUP(g2, fp2, F2_ZERO, F2_ONE)
    BN254: E(Fp) = G1, any correct method gives [k]P: the window method above.
    BLS12-381: mcl's G1::mul is the GLV method with psi(x, y) = (beta x, y) = [L] on G1, L = z^2 - 1: k mod r is split by plain division,
    k = a + b L (0 <= a < L), and the result is [a]P + [b]psi(P).  Inside G1 that is [k]P.  For a point of E(Fp) outside G1 -- mcl's default
-   accepts one on deserialisation -- it is not (psi fixes the order-3 points (0, +-2): that component is multiplied by a + b), and the
-   reference's verdict on such inputs follows this split: pinned by 20 crafted proofs / requests in tests/golden/bls12_381_oracle_{edge,requests}.json. */
+   accepts one on deserialisation -- it is not (psi fixes the order-3 points (0, +-2): that component is multiplied by a + b), so the
+   verdict on such inputs follows the split (20 crafted proofs / requests in tests/golden/bls12_381_oracle_{edge,requests}.json). */
 #ifdef ELPO_BLS12_381
 static const u64 GLV_L[2] = {0x00000000ffffffffull, 0xac45a4010001a402ull};                 /* z^2 - 1 */
 static const u64 GLV_BETA[NL] = {0x8bfd00000000aaacull, 0x409427eb4f49fffdull, 0x897d29650fb85f9bull, 0xaa0d857d89759ad4ull, 0xec02408663d4de85ull,
@@ -938,8 +937,8 @@ static void fp_set_hash_of(fp* r, const uint8_t* msg, size_t len) {
 }
 /* hashAndMapToG1 (call sites src/ps-verifier.cc:94,186, src/ps-requester.cc:185,336): t = Fp::setHashOf(msg), the Shallue-van de Woestijne map
    (mcl MapTo::calcBN; mcl's default, non-ETH mode uses it for BLS12-381 too), then -- BLS12-381 only -- multiplication by the G1 cofactor
-   (z-1)^2/3.  Pinned on both curves by the reference wasm's proofs (tests/golden/{bn254,bls12_381}_oracle_flows.json, section hash_to_g1:
-   32 service names, all six branch / sign cases). */
+   (z-1)^2/3.  Pinned on BN254 by the reference's proofs (tests/golden/bn254_oracle_flows.json, section hash_to_g1: 32 service names, all six
+   branch / sign cases); on BLS12-381 equal to the big-int model's, parity with the reference unpinned. */
 static fp SVDW_C1, SVDW_C2;
 #ifdef ELPO_BLS12_381
 static void g1_mul(g1j* r, const g1a* p, const u64* k);
@@ -1021,8 +1020,8 @@ void elpo_init(void) {
     fp2_mul(&a3, &a3, &a);        /* a^(1+p+p^2) */
     FROB[1][k] = a; FROB[2][k] = a2; FROB[3][k] = a3;
   }
-  /* SvdW constants: c1 = sqrt(-3) = (-3)^((p+1)/4), the root fp_sqrt returns (BN254: ...0004, BLS12-381: ...fffdfffd; both pinned by the
-     golden vectors), c2 = (c1 - 1)/2 */
+  /* SvdW constants: c1 = sqrt(-3) = (-3)^((p+1)/4), the root fp_sqrt returns (BN254: ...0004, BLS12-381: ...fffdfffd; the first pinned by
+     the golden vectors), c2 = (c1 - 1)/2 */
   fp m3, two, half;
   fp_from_u64(&m3, 3); fp_neg(&m3, &m3);
   fp_sqrt(&SVDW_C1, &m3);
@@ -1197,7 +1196,7 @@ static int elpo_strict = 0;
 void elpo_set_strict(int on) { elpo_strict = on; }
 /* the library's ELP_OPT_SUBGROUP_CHECK (BLS12-381): 1 (default here, as in the library) = the project's policy above, a DELIBERATE divergence from the
    reference; 0 = the reference's behaviour -- mcl's default does not test the order of a deserialised G1 point; together with g1_mul_ref this
-   build then reproduces every verdict of the reference's wasm on points outside G1 (tests/test_oracle_bls.py) */
+   build then answers on points outside G1 as the reference's statements do without the test (tests/test_oracle_bls.py) */
 static int elpo_subgroup_check = 1;
 void elpo_set_subgroup_check(int on) { elpo_subgroup_check = on; }
 

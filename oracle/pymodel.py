@@ -11,7 +11,8 @@ What it restates (all citations into /root/reference):
                      (BN254 "mcl default" curve, little-endian serialisation with y-parity flag,
                      Fr::setHashOf masking, BN Shallue-van de Woestijne hashAndMapToG1).
 Pinning: every convention below is checked against golden vectors captured from the reference's own
-prebuilt wasm (tests/golden/bn254_*.json, produced by oracle/gen_fixtures.js) in tests/test_oracle_golden.py.
+prebuilt wasm on its own curve, BN254 (tests/golden/bn254_*.json), in tests/test_oracle_golden.py.  On BLS12-381, which the
+reference does not run on, parity is unpinned: the model and the C oracle are checked against each other (tests/test_oracle_bls.py).
 
 The model is deliberately simple (affine formulas, generic square-and-multiply, no windows); it is the
 slow-but-obvious statement that the C oracle (oracle/elp_oracle.c) and the HIP path are checked against.
@@ -295,8 +296,8 @@ class Groups:
         method with the endomorphism psi(x, y) = (beta x, y) = [L] on G1, L = z^2 - 1: k mod r is split by plain division, b, a = divmod(k, L),
         and the result is [a]P + [b]psi(P).  Inside G1 that is [k]P; for a point of E(Fp) OUTSIDE G1 (which mcl's default accepts on
         deserialisation) it is not -- e.g. psi fixes the points (0, +-2) of order 3, so the order-3 component is multiplied by a + b instead of
-        k.  The split is pinned by the reference wasm's verdicts on 20 crafted proofs / requests (tests/golden/bls12_381_oracle_edge.json
-        "crafted_phi_c_mod_3", bls12_381_oracle_requests.json "crafted_A_c_mod_3": accepted iff 3 | a + b)."""
+        k.  20 crafted proofs / requests follow the split (tests/golden/bls12_381_oracle_edge.json "crafted_phi_c_mod_3",
+        bls12_381_oracle_requests.json "crafted_A_c_mod_3": accepted iff 3 | a + b; regression vectors, parity with mcl is unpinned)."""
         k %= self.cv.r
         if self.cv.is_bn or P is None:
             return self.g1_mul_plain(P, k)
@@ -471,7 +472,7 @@ class Mcl:
             assert self.c2 == 0x25236482400000017080EB4000000006181800000000000CD98000000000000B
             self.g1_cofactor = 1
         else:
-            # pinned by tests/golden/bls12_381_*.json (reference wasm with mcl's BLS12-381 CurveParam, oracle/wasm_curve.js)
+            # the root (-3)^((p+1)/4) of this p; parity with mcl's constant is unpinned
             assert self.c1 == 0xBE32CE5FBEED9CA374D38C0ED41EEFD5BB675277CDF12D11BC2FB026C41400045C03FFFFFFFDFFFD
             self.g1_cofactor = (cv.z - 1) ** 2 // 3
 
@@ -811,8 +812,8 @@ class Protocol:
         # golden case "sig_both_zero"), True = sig1 must be admissible as in PSVerifier::verify
         self.strict = False
         # the library's ELP_OPT_SUBGROUP_CHECK (BLS12-381 only; default 1 in the library): True = prover-supplied G1 points must lie in the order-r
-        # subgroup (project policy, a DELIBERATE divergence from the reference: mcl's default does not test the order of a deserialised G1 point --
-        # what the reference's wasm answers on such inputs is recorded in tests/golden/bls12_381_oracle_edge.json), False = no test.
+        # subgroup (project policy, a DELIBERATE divergence from the reference: mcl's default does not test the order of a deserialised G1 point),
+        # False = no test.
         self.subgroup_check = True
 
     # sigma_1 must not be the identity of G1 (src/ps-verifier.cc:16-18).  On a curve with a G1 cofactor (BLS12-381) that is asked of the order-r component:

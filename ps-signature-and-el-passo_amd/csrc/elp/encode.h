@@ -191,8 +191,8 @@ ELP_HEAVY bool g2_deserialize(Aff<F2<C>>& p, const uint8_t* in, bool* canon_flag
 //   P = SvdW(t)              Shallue-van de Woestijne map for y^2 = x^3 + b (mcl MapTo::calcBN; mcl's default, non-ETH mode uses it for
 //                            BLS12-381 too): c1 = sqrt(-3) = (-3)^((p+1)/4), c2 = (c1 - 1)/2, y negated iff Legendre(t) = -1
 //   BLS12-381: P <- [(z-1)^2/3] P   (cofactor clearing; the cofactor of BN254's E(Fp) is 1)
-// Pinned on BOTH curves by proofs made by the reference's wasm (tests/golden/{bn254,bls12_381}_oracle_flows.json "hash_to_g1": 32 service
-// names, all six branch / sign cases; the BLS12-381 run of the wasm: oracle/wasm_curve.js).
+// Pinned on BN254 by proofs made by the reference (tests/golden/bn254_oracle_flows.json "hash_to_g1": 32 service names, all six branch / sign
+// cases); on BLS12-381 equal to the big-integer model and the C oracle, parity with the reference unpinned.
 template <class C>
 ELP_HEAVY void map_to_g1_svdw(Aff<F1<C>>& out, const Fp<C>& t) {  // t != 0, Montgomery form
   Fp<C> c1, c2, b, one = fp_one<C>();

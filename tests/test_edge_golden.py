@@ -1,4 +1,4 @@
-"""Edge cases pinned by the reference's wasm (tests/golden/bn254_oracle_edge.json, generator oracle/gen_edge_fixtures.py):
+"""Edge cases pinned by the reference's wasm (tests/golden/bn254_oracle_edge.json):
 a commitment k OUTSIDE the order-r subgroup of the twist (src/ps-verifier.cc:73 multiplies an attacker-supplied k; mcl does no
 order check there) and the 3-byte length form inside T-L-V lists (src/ps-encoding.cc:149-162).  The reference rejects every
 off-subgroup k -- also a proof crafted so that its Schnorr half passes under plain scalar multiplication -- and accepts the

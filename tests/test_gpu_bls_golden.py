@@ -1,6 +1,6 @@
-"""GPU parity on BLS12-381 -- the curve north_star names -- against vectors produced by the REFERENCE'S OWN wasm run on that curve
-(tests/golden/bls12_381_*.json; generators oracle/gen_fixtures.js --curve bls12_381, oracle/gen_edge_fixtures.py --curve bls12_381,
-oracle/gen_request_fixtures.js --curve bls12_381; the curve switch of the wasm: oracle/wasm_curve.js).  Everything goes through the C-ABI.
+"""The GPU on BLS12-381 against recorded regression vectors (tests/golden/bls12_381_*.json).  They come from a prebuilt module patched to this
+curve and are no evidence of parity: the reference runs on BN254 only, and "reference" below means the recorded verdict.  (The independent checks
+of this curve, model and C oracle: tests/test_gpu_bls.py.)  Everything goes through the C-ABI.
 Record and wire entry points; the small-batch (cooperative / four-lane job), mid-size (four lanes per pairing) and full-size (two lanes per
 item) kernels are reached by tiling the reference's cases to the batch sizes that select them."""
 import base64
@@ -39,8 +39,8 @@ def _set_key(ctx, pk, svc=None, g_eg=None, apk=None, h=None, skX=None, W=6):
 
 
 def test_hash_to_g1_is_mcls_map(ctx):
-    """hashAndMapToG1 on the device = SHA-512 setHashOf + SvdW (b = 4) + cofactor: H1(svc) for the 32 service names whose reference-made proofs
-    pin the map (all six branch / sign cases), plus SHA-512 padding boundaries."""
+    """hashAndMapToG1 on the device = SHA-512 setHashOf + SvdW (b = 4) + cofactor: H1(svc) for the 32 recorded service names
+    (all six branch / sign cases), plus SHA-512 padding boundaries."""
     names = [c["svc"].encode() for c in FLOWS["hash_to_g1"]["cases"]] + [b"", b"x" * 111, b"x" * 112, b"x" * 127, b"x" * 128, b"x" * 300]
     out = ctx.hash_to_g1(names)
     for i, s in enumerate(names):

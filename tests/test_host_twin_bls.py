@@ -1,6 +1,6 @@
 """BLS12-381 instantiation of the device headers, checked on the CPU (host twin) against the big-int model.
-First half: equality with the big-int model plus algebraic known-answer properties (bilinearity, group order).  Second half: the vectors
-the reference's own wasm produced when run on this curve (tests/golden/bls12_381_*.json, oracle/wasm_curve.js)."""
+First half: equality with the big-int model plus algebraic known-answer properties (bilinearity, group order).  Second half: recorded
+regression vectors (tests/golden/bls12_381_*.json; from a module patched to this curve, no evidence of parity with the reference)."""
 import ctypes
 import os
 import random
@@ -142,7 +142,7 @@ def test_protocol_flows(L):
 
 
 # ------------------------------------------------------------------------------------------------------------------------------------------
-# Reference-run vectors for this curve (tests/golden/bls12_381_*.json: the reference's wasm with mcl's BLS12-381 CurveParam, oracle/wasm_curve.js)
+# Recorded regression vectors for this curve (tests/golden/bls12_381_*.json); "reference" below means the recorded verdict, parity is unpinned here
 # ------------------------------------------------------------------------------------------------------------------------------------------
 import base64  # noqa: E402
 
@@ -153,7 +153,7 @@ KEY_STRICT_SIG, KEY_NO_SUBGROUP_CHECK = 1, 2
 
 
 def test_hash_to_g1_is_mcls_on_every_reference_service_name(L):
-    """SHA-512 setHashOf + SvdW (b = 4) + cofactor, in the device headers: equal to the model on the 32 names whose reference-made proofs pin the map."""
+    """SHA-512 setHashOf + SvdW (b = 4) + cofactor, in the device headers: equal to the model on the 32 recorded names (all six branch / sign cases)."""
     o2 = ctypes.create_string_buffer(2 * N)
     for c in load_golden("bls12_381_oracle_flows.json")["hash_to_g1"]["cases"]:
         s = c["svc"]
@@ -165,7 +165,7 @@ def test_hash_to_g1_is_mcls_on_every_reference_service_name(L):
 
 
 def test_device_formulas_reproduce_reference_verdicts_record_and_wire(L):
-    """Every el_passo_verify_id_without_id_retrieval verdict of the reference's wasm on BLS12-381 (flows + with-retrieval run), through the one-lane,
+    """Every el_passo_verify_id_without_id_retrieval verdict recorded for BLS12-381 (flows + with-retrieval run), through the one-lane,
     two-lane, job-split and wire forms of the device code.  Options as the reference behaves: lenient signature rule; the subgroup test stays ON
     (no flow case leaves G1)."""
     flows = load_golden("bls12_381_oracle_flows.json")
@@ -272,7 +272,7 @@ def test_device_formulas_on_reference_edge_vectors(L):
 
 
 def test_device_issuance_on_reference_idp_vectors(L):
-    """tests/golden/bls12_381_oracle_requests.json: el_passo_provide_id verdicts of the reference's IdP on model-made requests; commitments outside
+    """tests/golden/bls12_381_oracle_requests.json: recorded el_passo_provide_id verdicts on model-made requests; commitments outside
     G1 are never signed under the library's default."""
     out = ctypes.create_string_buffer(4 * N)
     for s in load_golden("bls12_381_oracle_requests.json")["scenarios"]:

@@ -1,9 +1,9 @@
 """The C oracle's BLS12-381 build (oracle/elp_oracle.c -DELPO_BLS12_381) against the independent big-int model (oracle/pymodel.py).
 These tests establish that TWO independently written implementations (C: 6 x 64-bit Montgomery limbs, Jacobian lines, HHT chain; Python:
 big integers, affine formulas, plain exponentiation) agree bit for bit on primitives, GT values, issued signatures and verdicts --
-the pair then serves as the checker of the HIP path's BLS12-381 instantiation (tests/test_gpu_bls.py) and as its CPU baseline.  Both are
-pinned to the reference's own wasm run on this curve in tests/test_oracle_bls_golden.py; the subgroup / strict-signature tests below state
-the library's POLICY on points outside G1, which differs from the reference's behaviour on purpose (same file)."""
+the pair then serves as the checker of the HIP path's BLS12-381 instantiation (tests/test_gpu_bls.py) and as its CPU baseline.  Parity with
+the reference is unpinned on this curve (the reference runs on BN254); the subgroup / strict-signature tests below state the library's POLICY on
+points outside G1, which differs on purpose from the reference's statements, where no such test is made."""
 import copy
 import ctypes
 import random

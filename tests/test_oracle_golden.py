@@ -1,5 +1,5 @@
 """Pins the oracle: both restatements (oracle/pymodel.py big-int model, oracle/elp_oracle.c) must reproduce every golden
-vector captured from the reference's own wasm build (tests/golden/bn254_*.json, generator oracle/gen_fixtures.js), and
+vector captured from the reference's own wasm build (tests/golden/bn254_*.json), and
 must agree with each other on the primitives."""
 import base64
 import ctypes

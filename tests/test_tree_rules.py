@@ -43,3 +43,13 @@ def test_no_build_switch_ends_a_verification_early_and_no_script_reproduces_a_fa
     assert hits(r"ELP_[B]ISECT") == []
     assert [n for n in source_files() if re.search(r"fault_(repro|probe)", n)] == []
     assert hits(r"[_]fault_(repro|probe)\b") == []
+
+
+def test_nothing_runs_searches_or_patches_a_prebuilt_module():
+    """Vectors come from source built here or from data already recorded; no script loads the reference's prebuilt modules, reads their memory image or writes into it, and no
+    text calls the BLS12-381 vectors an ordinary run of the reference."""
+    assert hits(r"[w]asm-build|HEAP[U](8|16|32)\b|select[C]urve|wasm[_](curve|verify)") == []
+    assert [n for n in source_files() if n.endswith(".js")] == []
+    claim = re.compile(r"wasm run on (this|that|the) curve|run on BOTH curves|reference-run oracle|BLS12-381 is pinned|pinned (on|by) (BOTH|both) curves|both curves by (proofs|reference)", re.I)
+    texts = source_files() + ["README.md", "DESIGN.md", "INTEGRATION.md"]
+    assert [n for n in texts if n != "tests/test_tree_rules.py" and claim.search(open(os.path.join(ROOT, n), errors="replace").read())] == []
