@@ -53,3 +53,26 @@ def test_nothing_runs_searches_or_patches_a_prebuilt_module():
     claim = re.compile(r"wasm run on (this|that|the) curve|run on BOTH curves|reference-run oracle|BLS12-381 is pinned|pinned (on|by) (BOTH|both) curves|both curves by (proofs|reference)", re.I)
     texts = source_files() + ["README.md", "DESIGN.md", "INTEGRATION.md"]
     assert [n for n in texts if n != "tests/test_tree_rules.py" and claim.search(open(os.path.join(ROOT, n), errors="replace").read())] == []
+
+
+def test_no_source_names_a_write_through_the_scalar_data_cache():
+    """GPU code writes through vector stores only, and the tree says so to a reader of its text: no source, script or build file names a scalar store, a scalar atomic, or the
+    write-back and discard of that cache."""
+    assert hits(r"\bs_(buffer_|scratch_)?(store|atomic)_|\bs_d""cache_(wb|discard)") == []
+
+
+def test_long_branch_scanner_accepts_only_saves_that_a_compiled_function_makes(tmp_path):
+    """The return address counts as saved by a lane write or a copy into other scalar registers, before the first clobbering s_getpc_b64; anything else in that place -- a vector
+    store of unrelated registers, a scalar one of s[30:31] -- leaves the function reported."""
+    import sys
+    sys.path.insert(0, os.path.join(ROOT, "tools"))
+    import check_long_branch as clb
+    body = "\tv_add_u32_e32 v0, v1, v2\n" * 4
+    far = "\ts_getpc_b64 s[30:31]\n.Lpost_getpc1:\n\ts_add_u32 s30, s30, 12\n\ts_addc_u32 s31, s31, 0\n\ts_setpc_b64 s[30:31]\n"
+    listing = "".join(name + ":\n" + before + body + far + body + "\ts_setpc_b64 s[30:31]\n" for name, before in (
+        ("saved_in_lanes", "\tv_writelane_b32 v40, s30, 0\n\tv_writelane_b32 v40, s31, 1\n"), ("saved_as_pair", "\ts_mov_b64 s[34:35], s[30:31]\n"),
+        ("saved_in_halves", "\ts_mov_b32 s34, s30\n\ts_mov_b32 s35, s31\n"), ("vector_store", "\tscratch_store_dword off, v40, s33\n"),
+        ("scalar_store", "\ts_" + "store_dwordx2 s[30:31], s[4:5], 0x0\n")))
+    p = tmp_path / "listing.s"
+    p.write_text(listing)
+    assert [b[0] for b in clb.scan(str(p))] == ["vector_store", "scalar_store"]

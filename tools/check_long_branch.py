@@ -4,8 +4,8 @@ A device FUNCTION (not a kernel) returns with `s_setpc_b64 s[30:31]`.  When its 
 branches as `s_getpc_b64 sN ; s_add_u32 ; s_addc_u32 ; s_setpc_b64 sN` with a scavenged SGPR pair -- and under scalar-register pressure ROCm 7.2.0's hipcc picks
 s[30:31] itself in a LEAF function, which never saved it: the first far branch taken destroys the return address.  This script reads hipcc assembly listings
 (-save-temps) or `llvm-objdump -d` output and reports every function that (a) is not a kernel, (b) writes s[30:31] with s_getpc_b64 and (c) has not saved s30
-BEFORE the first such write (v_writelane_b32 ..., s30, ... / s_mov_b64 ..., s[30:31] / a scalar or vector store of s[30:31] to memory): a save after the clobbering
-instruction would store the clobbered value.
+BEFORE the first such write (v_writelane_b32 ..., s30, ... / s_mov_b64 ..., s[30:31] / s_mov_b32 ..., s30): a save after the clobbering instruction would keep the
+clobbered value.  Any other way of saving the pair is not recognised and leaves the function reported.
     python tools/check_long_branch.py <file.s | objdump.txt> [...]      exit code 1 if a hazardous function is found."""
 import re
 import sys
@@ -23,9 +23,8 @@ def scan(path):
             return                                     # a kernel, or no return through s[30:31]
         far = len(re.findall(r"s_getpc_b64 s\[30:31\]", body))
         first = re.search(r"s_getpc_b64 s\[30:31\]", body)
-        # the return address counts as saved only if the save precedes the first clobbering s_getpc_b64 (spills through memory included)
-        saved = first and re.search(r"v_writelane_b32 v\d+, s30\b|s_mov_b64 s\[\d+:\d+\], s\[30:31\]|s_store_dwordx2 s\[30:31\]|s_mov_b32 s\d+, s30\b",
-                                    body[:first.start()])
+        # the return address counts as saved only if the save precedes the first clobbering s_getpc_b64
+        saved = first and re.search(r"v_writelane_b32 v\d+, s30\b|s_mov_b64 s\[\d+:\d+\], s\[30:31\]|s_mov_b32 s\d+, s30\b", body[:first.start()])
         if far and not saved:
             bad.append((name, far, len(body.encode())))
 
