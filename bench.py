@@ -398,7 +398,7 @@ def aggregated_section(ctx, wl, synth, dev, mask, H, B):
 
     # the multi-stream measurements come FIRST, while the process has not yet run a 2^20-item launch on its default stream (see run_child_section)
     # sustained: the 16 distinct batches of 65 536, twice over, alternating between two streams (aggregated) / back to back on one stream (per item)
-    sa, sb = torch.cuda.Stream(device=dev), torch.cuda.Stream(device=dev, priority=-1)      # the second one from the other priority pool: surely another hardware queue
+    sa, sb = torch.cuda.Stream(device=dev), torch.cuda.Stream(device=dev)
     nbat = NT // B
     # Exactly two side streams.  What overlaps is the TAIL of one batch with the tail of the other (a per-item kernel holds every SIMD's registers, so a tail cannot run
     # beside it: profiles/r04_agg_two_stream_timeline.txt, r06_agg_two_stream_timeline.txt), and only if the two streams sit on two hardware queues.  More streams do not help and run into the runtime's

@@ -76,3 +76,8 @@ def test_long_branch_scanner_accepts_only_saves_that_a_compiled_function_makes(t
     p = tmp_path / "listing.s"
     p.write_text(listing)
     assert [b[0] for b in clb.scan(str(p))] == ["vector_store", "scalar_store"]
+
+
+def test_every_stream_has_the_default_priority():
+    """Streams of different priorities are not mixed: no stream, process group or graph asks for one."""
+    assert hits(r"\bpriority\s*=|high_[p]riority|Stream\w*With[P]riority") == []
