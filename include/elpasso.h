@@ -53,17 +53,17 @@ int elp_field_bytes(int curve);               /* F */
  *   ELP_OPT_SUBGROUP_CHECK on, a sig1 outside G1.  The reference has no such test in el_passo_verify_id (src/ps-verifier.cc:133-137): it accepts
  *   sig1 = sig2 = infinity with a self-made NIZK (golden case "sig_both_zero"), and the same statements evaluated on BLS12-381 accept
  *   (sig1, sig2) = (T, O) with T of order 3 as well as sig1 + T -- universal forgeries, since a point whose order divides the cofactor pairs to 1
- *   with everything.  0 = the reference's statements without the test (on BLS12-381 together with ELP_OPT_SUBGROUP_CHECK = 0).  elp_ps_verify_batch always rejects sig1 = infinity as PSVerifier::verify does (src/ps-verifier.cc:16-18) and, with the subgroup check on,
- *   sig1 outside G1.
+ *   with everything.  0 = the reference's statements without the test (on BLS12-381 together with ELP_OPT_SUBGROUP_CHECK = 0).
+ *   elp_ps_verify_batch always rejects sig1 = infinity as PSVerifier::verify does (src/ps-verifier.cc:16-18) and, with the subgroup check on, sig1
+ *   outside G1.
  * ELP_OPT_SUBGROUP_CHECK (default 1; BLS12-381 only -- E(Fp) of BN254 has prime order): the prover-supplied G1 points of a proof or request -- phi, E1,
  *   E2, the commitment A of el_passo_provide_id, and sig1 where the strict rule applies -- must lie in the order-r subgroup, otherwise the item is
  *   rejected.  A DELIBERATE divergence from the reference: mcl's default does not test the order of a deserialised G1 point.  Its statements without the test,
  *   as the big-integer model and the C oracle evaluate them: phi + T with an honest transcript: rejected; a crafted phi + T3 or A + T3 with 3 | c:
  *   accepted iff a GLV split c = a + b (z^2 - 1) has 3 | a + b (about one in three); sig1 / sig2 + T: accepted.  phi is
  *   the user's pseudonym and (E1, E2) the identity-retrieval token: a small-order component would give one user several pseudonyms or an undecryptable
- *   token, hence the check.  0 = no check, on EVERY path: for inputs the caller has validated.  The sig1 cases are then accepted;
- *   the verdict on a phi / E1 / E2 / A outside G1 is implementation-defined (the device's GLV split is not mcl's), and (sig1 of order 3,
- *   sig2 = O) verifies.
+ *   token, hence the check.  0 = no check, on EVERY path: for inputs the caller has validated.  The sig1 cases are then accepted; the
+ *   verdict on a phi / E1 / E2 / A outside G1 is implementation-defined (the device's GLV split is a lattice split), and (sig1 of order 3, sig2 = O) verifies.
  *
  * KERNEL SELECTION (verdicts identical):
  * ELP_OPT_PAIRED_LAYOUT: 0 = one lane per item; 1 = two lanes per item (the Fp2 tower split over a lane pair; BN254 builds); 2 (default) = by batch
@@ -148,7 +148,8 @@ size_t elp_msm_workspace_bytes(int curve, int group, size_t n);
 int elp_g1_msm_dev(elp_ctx* ctx, void* stream, size_t n, const void* d_points, const void* d_scalars, void* d_workspace, void* d_out);
 int elp_g2_msm_dev(elp_ctx* ctx, void* stream, size_t n, const void* d_points, const void* d_scalars, void* d_workspace, void* d_out);
 /* hashAndMapToG1 (src/ps-verifier.cc:94,186; src/ps-requester.cc:185,336) as mcl evaluates it: Fp::setHashOf (SHA-256 on BN254, SHA-512 on BLS12-381),
- * the Shallue-van de Woestijne map, and on BLS12-381 the cofactor (z-1)^2/3; pinned by reference-made proofs on BN254, by the model and the C oracle on BLS12-381. msgs concatenated, offsets[n+1]. */
+ * the Shallue-van de Woestijne map, and on BLS12-381 the cofactor (z-1)^2/3; pinned by reference-made proofs on BN254, equal to the model and the C oracle on
+ * BLS12-381. msgs concatenated, offsets[n+1]. */
 int elp_hash_to_g1(elp_ctx* ctx, size_t n, const uint8_t* msgs, const uint32_t* offsets, uint8_t* out);
 /* pairing(GT&, G1, G2) (src/ps-verifier.cc:32-33) */
 int elp_pairing(elp_ctx* ctx, size_t n, const uint8_t* g1, const uint8_t* g2, uint8_t* gt);
