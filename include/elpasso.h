@@ -100,10 +100,15 @@ int elp_field_bytes(int curve);               /* F */
  *   0 = the interpreter and the one-lane product tree keep these jobs.  Measurements: profiles/r06_pair16.md.
  * ELP_OPT_FAULT_INJECT (default 0; test hook for callers' error paths): the next `value` calls of elp_verify_id_batch_submit on this context fail with
  *   ELP_ERR_STATE before anything is queued.  No other entry point consumes or honours the counter.
+ * ELP_OPT_LAUNCH_STREAM (default 0): the kernels of the host-buffer and pipelined calls of ALL contexts of a device run on one stream (copies keep a stream per
+ *   context).  1 = on the device's second launch stream, for a second context whose batches are to overlap the first one's: two contexts on one GPU then
+ *   reach 4.0 instead of 3.3 M el_passo_verify_id/s with pipelined batches of 65 536.  There are two and no more, because private memory is provisioned per hardware queue (8 GiB
+ *   each for the largest kernels) and a process that spreads them over four queues has its next dispatch aborted for want of it; the same holds for the
+ *   streams a caller hands to the _dev entry points.  Waits for what the context has queued, then switches.
  */
 enum { ELP_OPT_STRICT_SIGNATURE = 1, ELP_OPT_PAIRED_LAYOUT = 2, ELP_OPT_TABLE_WORKSPACE = 3, ELP_OPT_SPLIT_PHASES = 4, ELP_OPT_SUBGROUP_CHECK = 5,
        ELP_OPT_COOP_PAIRING = 6, ELP_OPT_COALESCED_RECORDS = 7, ELP_OPT_STREAM_OVERLAP = 8, ELP_OPT_FAULT_INJECT = 9, ELP_OPT_PAIR4 = 10, ELP_OPT_WIRE_DECODE = 11,
-       ELP_OPT_AGG_TWO_PER_LANE = 12, ELP_OPT_PAIR16 = 13 };
+       ELP_OPT_AGG_TWO_PER_LANE = 12, ELP_OPT_PAIR16 = 13, ELP_OPT_LAUNCH_STREAM = 14 };
 int elp_set_option(elp_ctx* ctx, int option, int value);
 const char* elp_version(void);
 

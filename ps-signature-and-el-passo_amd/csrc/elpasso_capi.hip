@@ -79,6 +79,36 @@ int elp_device_count(void) {
   return ndev;
 }
 
+// The launch streams of a device, shared by its contexts and kept for the life of the process: one for all of them, a second one on request (ELP_OPT_LAUNCH_STREAM).
+// The runtime provisions private memory per hardware queue and for a full device whatever the grid -- frame x 64 lanes x 32 wave slots per compute unit, 8.04 GiB for the 16 464 B
+// of k_verify_id_agg on 256 units (measured: a second context with a stream of its own added 8.04 GiB, on a shared one 12 MiB) -- and keeps it when the stream is gone.
+// Streams are dealt to four queues, with 4 GiB per XCD = 32 GiB of such space between them: four queues that have each run a kernel with a frame of 16 KB leave none, and the next
+// dispatch that needs a larger block aborts its queue.  Copy streams (pstream) stay per context.
+static hipError_t launch_stream(int device, int which, hipStream_t* out) {
+  static std::mutex mu;
+  static std::vector<hipStream_t> streams;
+  std::lock_guard<std::mutex> g(mu);
+  const size_t slot = 2 * (size_t)device + (size_t)which;
+  if (slot >= streams.size()) streams.resize(slot + 1, nullptr);
+  hipStream_t& s = streams[slot];
+  if (s) {
+    const hipError_t e = hipStreamQuery(s);                 // after a device reset by the caller the handle is stale: a new stream then
+    if (e != hipSuccess && e != hipErrorNotReady) {
+      (void)hipGetLastError();
+      s = nullptr;
+    }
+  }
+  if (!s) {
+    const hipError_t e = hipStreamCreate(&s);
+    if (e != hipSuccess) {
+      s = nullptr;
+      return e;
+    }
+  }
+  *out = s;
+  return hipSuccess;
+}
+
 int elp_init(int curve, int device, elp_ctx** out) {
   if (!out) return ELP_ERR_ARG;
   *out = nullptr;
@@ -110,7 +140,7 @@ int elp_init(int curve, int device, elp_ctx** out) {
   if (const char* e = getenv("ELP_VTAB")) c->use_vtab = strcmp(e, "0") != 0;                                         // A/B runs: tables of multiples in private memory
   hipDeviceProp_t prop;
   if (hipGetDeviceProperties(&prop, device) == hipSuccess && prop.multiProcessorCount > 0) c->simds = 4 * prop.multiProcessorCount;
-  if (hipStreamCreate(&c->stream) != hipSuccess) {
+  if (launch_stream(device, 0, &c->stream) != hipSuccess) {
     delete c;
     return ELP_ERR_HIP;
   }
@@ -156,8 +186,7 @@ void elp_destroy(elp_ctx* c) {
   if (c->jstream) (void)hipStreamDestroy(c->jstream);
   for (int i = 0; i < 4; i++)
     if (c->jev[i]) (void)hipEventDestroy(c->jev[i]);
-  (void)hipStreamDestroy(c->stream);
-  delete c;
+  delete c;                                               // the launch stream belongs to the device
 }
 
 const char* elp_last_error(const elp_ctx* c) { return c ? c->err.c_str() : "null context"; }
@@ -194,6 +223,13 @@ int elp_set_option(elp_ctx* c, int option, int value) {
       c->pair16 = value ? 1 : 0;
       c->pair16_max = value > 1 ? (size_t)value : 4096;
       return ELP_OK;
+    case ELP_OPT_LAUNCH_STREAM: {
+      if (value < 0 || value > 1) return ELP_ERR_ARG;
+      HIPCHK(c, hipSetDevice(c->device));
+      HIPCHK(c, hipStreamSynchronize(c->stream));           // what this context has queued is done before it moves
+      HIPCHK(c, launch_stream(c->device, value, &c->stream));
+      return ELP_OK;
+    }
     case ELP_OPT_SPLIT_PHASES:
       if (value < 0 || value > 3) return ELP_ERR_ARG;
       c->split = value;

@@ -2,6 +2,8 @@
 
 #include <string.h>
 
+#include <algorithm>
+
 static bool g_strict_signature = true;
 void elpSetStrictSignature(bool strict) { g_strict_signature = strict; }
 
@@ -68,7 +70,8 @@ ElpShardSet::ElpShardSet(const PSPubKey& pk, const std::vector<int>& devices, in
   std::vector<std::thread> th;
   auto make = [&](size_t r) {
     try {
-      keys_[r] = std::make_shared<ElpKey>(pk, devices[r], window_bits);
+      const int earlier = (int)std::count(devices.begin(), devices.begin() + (long)r, devices[r]);      // an ordinal that repeats: its contexts overlap on two streams
+      keys_[r] = std::make_shared<ElpKey>(pk, devices[r], window_bits, earlier & 1);
     } catch (...) {
       errs[r] = std::current_exception();
     }
@@ -80,13 +83,19 @@ ElpShardSet::ElpShardSet(const PSPubKey& pk, const std::vector<int>& devices, in
     if (e) std::rethrow_exception(e);
 }
 
-ElpKey::ElpKey(const PSPubKey& pk, int device, int window_bits) {
+ElpKey::ElpKey(const PSPubKey& pk, int device, int window_bits, int launch_stream) {
   if (pk.Yi.size() != pk.YYi.size() || pk.Yi.empty() || pk.Yi.size() > 62) throw std::runtime_error("ElpKey: bad public key shape");
   nattr_ = pk.Yi.size();
   if (device < 0) device = g_default_device >= 0 ? g_default_device : mcl::bls12::defaultDevice();
   if (window_bits < 0) window_bits = g_default_window;
   elpCheck(nullptr, elp_init(curveId(), device, &ctx_), "elp_init");      // the curve initPairing() selected for the process
   elp_set_option(ctx_, ELP_OPT_STRICT_SIGNATURE, g_strict_signature ? 1 : 0);
+  if (launch_stream && elp_set_option(ctx_, ELP_OPT_LAUNCH_STREAM, launch_stream) != ELP_OK) {
+    std::string msg = elp_last_error(ctx_);
+    elp_destroy(ctx_);
+    ctx_ = nullptr;
+    throw std::runtime_error("ElpKey: no second launch stream: " + msg);
+  }
   const size_t S1 = G1::size(), S2 = G2::size();
   std::vector<uint8_t> yi(S1 * nattr_), yyi(S2 * nattr_);
   for (size_t i = 0; i < nattr_; i++) {

@@ -13,7 +13,7 @@
 class ElpKey {
  public:
   // device / window_bits < 0: the process defaults (elpSetDefaults; initially the device initPairing() selected and the library's window width)
-  explicit ElpKey(const PSPubKey& pk, int device = -1, int window_bits = -1);
+  explicit ElpKey(const PSPubKey& pk, int device = -1, int window_bits = -1, int launch_stream = 0);
   ~ElpKey();
   ElpKey(const ElpKey&) = delete;
   ElpKey& operator=(const ElpKey&) = delete;
@@ -60,7 +60,7 @@ int elpDefaultWindowBits();
 int elpDefaultSideWindowBits();      // PSSigner / PSRequester
 
 // Several contexts of the same public key -- one per entry of `devices` (an ordinal may repeat: several contexts on one GPU) -- each with its own
-// host thread and HIP stream while a batch is in flight.  Batches are cut into contiguous shards, shard r of N taking items
+// host thread while a batch is in flight; contexts on one GPU take its two launch streams in turn.  Batches are cut into contiguous shards, shard r of N taking items
 // [r n / N, (r + 1) n / N); nothing is exchanged between shards, the per-shard counts are summed by the caller.  Set-up (tables) runs in parallel.
 class ElpShardSet {
  public:

@@ -23,6 +23,7 @@ OPT_PAIR4 = 10
 OPT_WIRE_DECODE = 11
 OPT_AGG_TWO_PER_LANE = 12
 OPT_PAIR16 = 13
+OPT_LAUNCH_STREAM = 14
 
 _c = ctypes
 _u8p = _c.c_void_p
@@ -210,6 +211,10 @@ class Context:
     def set_agg_two_per_lane(self, mode):
         """ELP_OPT_AGG_TWO_PER_LANE: aggregated verification with two proofs per lane (0 never -- the default --, 1 where it saves rounds of lanes, 2 always)."""
         self._chk(self.lib.elp_set_option(self.h, OPT_AGG_TWO_PER_LANE, int(mode)))
+
+    def set_launch_stream(self, which):
+        """ELP_OPT_LAUNCH_STREAM: 0 (default) = the launch stream that all contexts of the device share, 1 = the device's second one."""
+        self._chk(self.lib.elp_set_option(self.h, OPT_LAUNCH_STREAM, int(which)))
 
     def set_split_phases(self, on):
         """ELP_OPT_SPLIT_PHASES (default 0): 1 / 2 = one-lane-per-item verify_id as phase-split kernels (NIZK jobs, then the pairing); identical results."""
