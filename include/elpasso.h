@@ -67,8 +67,8 @@ int elp_field_bytes(int curve);               /* F */
  *
  * KERNEL SELECTION (verdicts identical):
  * ELP_OPT_PAIRED_LAYOUT: 0 = one lane per item; 1 = two lanes per item (the Fp2 tower split over a lane pair; BN254 builds); 2 (default) = by batch
- *   size: two lanes when the last round of 64 x SIMDs items would be at most half full and always on BLS12-381, one lane otherwise.  On BLS12-381 the
- *   main kernel of elp_verify_id_batch_aggregated[_dev] follows the option too (two lanes unless the value is 0; on BN254 it is a one-lane kernel).
+ *   size: two lanes when the last round of 64 x SIMDs items would be at most half full and always on BLS12-381, one lane otherwise.  The main
+ *   kernel of elp_verify_id_batch_aggregated[_dev] does not follow the option: two lanes on BLS12-381, one lane on BN254.
  * ELP_OPT_TABLE_WORKSPACE (default 1): the per-item tables of the variable-base multiplications live in a launch workspace in device memory (3 KB per
  *   item, see the *_dev entry points) instead of the lanes' private memory; 0 saves the memory at a few per cent of throughput.
  * ELP_OPT_SPLIT_PHASES (default 0): 1 = the one-lane el_passo_verify_id as two kernels (NIZK half as independent jobs, then the pairing check; BN254);

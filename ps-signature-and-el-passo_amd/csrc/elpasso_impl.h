@@ -2124,7 +2124,6 @@ struct elp_ctx {
   int mid_two_launches = 0;      // experiments (ELP_PAIR4_TWO_LAUNCHES=1): the mid-size path as k_vid_nizk4 then k_pair4 instead of the one launch k_vid_mid
   unsigned long long* wire_mask_host = nullptr;      // page-locked slot for the decoded wire path's 16-byte read-back
   int wire_decode = 1;           // ELP_OPT_WIRE_DECODE: wire batches of up to 16 384 messages are decoded into records and take the small / mid-size record paths
-  int agg_paired = 1;         // BLS12-381 with the two-lane layout allowed: the main kernel of aggregated verification on lane pairs (k_verify_id_agg_paired; ELP_AGG_PAIRED=0 for A/B runs)
   int agg_two = 0;            // ELP_OPT_AGG_TWO_PER_LANE: aggregated batches put two items on a lane (0 = never -- the default: 2 % at best, and the kernel's larger frame makes the runtime re-provision scratch --, 1 = where it saves rounds of lanes, 2 = always)
   int pair16 = 0;                // ELP_OPT_PAIR16 (set by elp_init): PS verifications of at most pair16_max items run the pairing check on one 16-lane row per item
   int pair16_tail = 1;           // the closing step of aggregated verification on one row (k_agg_final16; both curves: 1.02 against 1.19 ms on BN254, 2.21 against 2.63 ms on BLS12-381)
@@ -2822,8 +2821,10 @@ int elp_verify_id_batch_aggregated_dev_t(elp_ctx* c, void* stream_, size_t n, co
     const size_t round = (size_t)64 * c->simds, r1 = (n + round - 1) / round, r2 = (n + 2 * round - 1) / (2 * round);
     two_per_lane = c->agg_two == 2 || (c->agg_two == 1 && 189 * r2 < 100 * r1);
   }
-  bool paired_main = false;                                // BLS12-381: the main kernel on lane pairs (32 items per wave)
-  if constexpr (PairedBuild<C>::value && !C::IS_BN) paired_main = c->paired != 0 && c->agg_paired != 0;
+  // BLS12-381: the main kernel always on lane pairs (32 items per wave).  One lane per item took 75.6 against 41.0 ms at 65 536 proofs, and its private frame of 25 KB (12.4 GiB
+  // for a full device) does not fit beside the blocks of the process's other queues (launch_stream in elpasso_capi.hip): such a dispatch aborted its queue.
+  constexpr bool paired_main = !C::IS_BN;
+  static_assert(C::IS_BN || PairedBuild<C>::value, "the curve's aggregated main kernel exists on lane pairs only");
   const size_t nw = paired_main ? (size_t)((2 * n + ELP_BLOCK - 1) / ELP_BLOCK) : two_per_lane ? grid_for((n + 1) / 2) : grid_for(n);      // waves = per-wave Miller products
   const size_t nw2 = (nw + 31) / 32;                                                          // the larger of the two product trees' first level (rows: 32 values per workgroup)
   auto al = [](size_t x) { return (x + 255) & ~(size_t)255; };
@@ -2865,17 +2866,17 @@ int elp_verify_id_batch_aggregated_dev_t(elp_ctx* c, void* stream_, size_t n, co
     return ELP_ERR_STATE;
   }
   KeyCtx<C> key = make_key_ws<C>(c, stream, (size_t)nw * ELP_BLOCK);
-  if (paired_main) {
-    if constexpr (PairedBuild<C>::value && !C::IS_BN)
-      launch_verify_id_agg_paired<C>(c, stream, n, d_records, words, mask, retr, d_ad, d_ad_off, ad_len, seed, ws + o_flags, ws + o_delta, ws + o_sig2, ws + o_f1);
-  } else if (two_per_lane)
+  if constexpr (paired_main) {
+    launch_verify_id_agg_paired<C>(c, stream, n, d_records, words, mask, retr, d_ad, d_ad_off, ad_len, seed, ws + o_flags, ws + o_delta, ws + o_sig2, ws + o_f1);
+  } else if (two_per_lane) {
     hipLaunchKernelGGL((k_verify_id_agg2<C>), dim3(nw), dim3(ELP_BLOCK), 0, stream, key, (const u32*)d_records, words, (u64)mask, retr,
                        (const uint8_t*)d_ad, (const u32*)d_ad_off, (u32)ad_len, seed, ws + o_flags, (u32*)(ws + o_delta), (u32*)(ws + o_sig2),
                        (Fp12<C>*)(ws + o_f1), n);
-  else
+  } else {
     hipLaunchKernelGGL((k_verify_id_agg<C>), dim3(nw), dim3(ELP_BLOCK), 0, stream, key, (const u32*)d_records, words, (u64)mask, retr,
                        (const uint8_t*)d_ad, (const u32*)d_ad_off, (u32)ad_len, seed, ws + o_flags, (u32*)(ws + o_delta), (u32*)(ws + o_sig2),
                        (Fp12<C>*)(ws + o_f1), n);
+  }
   key.vtab = nullptr;   // the kernels below do not advance the pointer to their lane (the rare per-item fallback keeps its tables in private memory)
   // The two halves of the tail are independent -- the product of the per-wave Miller values (nw -> nw2 -> 1) and S2 = sum d_i sig2_i (Pippenger) -- and
   // neither fills the chip: with ELP_OPT_STREAM_OVERLAP the product runs on the context's second stream beside the sum.

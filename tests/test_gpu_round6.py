@@ -145,8 +145,8 @@ def test_aggregated_product_tree_on_rows_vs_oracle(gpu_ctx, elp):
     wave counts exercise a lone value (1 wave), one row (8), two rows (9), a full workgroup plus two values (34), plus a row and one (41), and a second level of five
     values (129) -- (a) bad items fail the NIZK half only: the batch equation must HOLD, which it does only if the product is exact; (b) two swapped sig2: it must FAIL
     and the per-item fallback decide.  Every verdict against the C oracle (elpo_verify_id_batch, src/ps-verifier.cc:37-138) and against the one-lane product tree
-    (ELP_OPT_PAIR16 = 0).  The BLS12-381 build of the same kernel at 34 and 41 waves, under both main kernels of that curve: on lane pairs (k_verify_id_agg_paired, the
-    default: 32 items per wave, so twice the waves) and on one lane per item (ELP_AGG_PAIRED=0)."""
+    (ELP_OPT_PAIR16 = 0).  The BLS12-381 build of the same kernel at 34 and 41 waves, twice: its main kernel is on lane pairs (k_verify_id_agg_paired, 32 items per
+    wave, so twice the waves) whatever ELP_AGG_PAIRED says -- the one-lane kernel that it once selected is out of the library."""
     import os
     from elp_testlib import oracle_bls
     seed = bytes(range(32, 64))
