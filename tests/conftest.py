@@ -3,6 +3,11 @@ import sys
 
 import pytest
 
+# One process runs the whole GPU suite, with many contexts and streams.  Private memory is provisioned per hardware queue and kept; two queues fit whatever they run
+# (test_private_frames.py), four do not.  Set before HIP starts.
+if not 1 <= int(os.environ.get("GPU_MAX_HW_QUEUES", "4")) <= 2:
+    os.environ["GPU_MAX_HW_QUEUES"] = "2"
+
 ROOT = os.path.abspath(os.path.join(os.path.dirname(__file__), ".."))
 for p in (ROOT, os.path.join(ROOT, "tests")):
     if p not in sys.path:
