@@ -48,7 +48,8 @@ print("DONE", flush=True)
 
 def test_a_second_context_needs_no_second_block_of_private_memory():
     """In a process of its own (a fresh runtime): the second context's first aggregated verification adds its tables and workspaces (some tens of MiB), not 8 GiB."""
-    r = subprocess.run([sys.executable, "-c", CHILD % ROOT], capture_output=True, text=True, timeout=100, cwd=ROOT)
+    r = subprocess.run([sys.executable, "-c", CHILD % ROOT], capture_output=True, text=True, timeout=100, cwd=ROOT,
+                       env=dict(os.environ, GPU_MAX_HW_QUEUES="4"))          # HIP's own default: the streams of two contexts would land on two queues
     assert r.returncode == 0 and "DONE" in r.stdout, r.stdout + r.stderr
     one, two, three = (float(x) for x in r.stdout.split("MIB")[1].split()[:3])
     print("used after one context %.0f MiB, after two %.0f, after the first again %.0f" % (one, two, three))
